@@ -40,17 +40,13 @@ own = False
 _DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16}
 
 
-_package = None  # imported once, as a program does
-
-
 def _kernels():
-    global _package
-    if _package is None:
-        sys.path.insert(0, str(Path.cwd() / "bdh-gpu-fast_amd"))
-        import kernels
+    pkg = str(Path.cwd() / "bdh-gpu-fast_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    import kernels
 
-        _package = kernels
-    return _package
+    return kernels
 
 
 # ------------------------------------------------------------------- cases
