@@ -39,7 +39,10 @@ struct Where {
 const at::Tensor* tensor(PyObject* o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
 
 bool here(const at::Tensor& t, const Where& w) { return t.is_cuda() && t.get_device() == w.device; }
-bool needs_grad(const at::Tensor& t) { return t.requires_grad() && c10::GradMode::is_enabled(); }
+// Gradients or a forward-mode tangent, which a result would lose (level 0 is autograd's only one).
+bool needs_grad(const at::Tensor& t) {
+  return (t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(0).defined();
+}
 
 bool unit(const at::Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1; }
 

@@ -24,6 +24,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import hip_attn
 
@@ -163,10 +164,15 @@ def _float_rows(name: str, t: torch.Tensor) -> None:
 
 
 def _no_grad(name: str, *ts: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled():
-        for t in ts:
-            if t is not None and t.requires_grad:
-                raise ValueError(f"{name} has no backward: call it under torch.no_grad() or detach its inputs")
+    """Operands, outputs among them, that need gradients or carry a forward-mode tangent."""
+    grad = torch.is_grad_enabled()
+    for t in ts:
+        if t is None:
+            continue
+        if grad and t.requires_grad:
+            raise ValueError(f"{name} has no backward: call it under torch.no_grad() or detach its operands")
+        if unpack_dual(t).tangent is not None:  # (no_grad does not put these off)
+            raise ValueError(f"{name} has no forward-mode derivative: call it on the primal tensors")
 
 
 def _same(name: str, m: Mx4, t: torch.Tensor) -> None:

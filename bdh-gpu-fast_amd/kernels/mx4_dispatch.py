@@ -6,8 +6,8 @@ binding, which takes arguments that need no preparation; the checks after it say
 what is wrong with others, or prepare them.  The backends are those of the
 attention (``BDH_ATTN_IMPL``): ``hip`` runs the gfx950 kernels, ``eager`` torch
 operations, on any device.  Both give the same codes; products differ in
-summation order.  Nothing here has a backward: inputs that need gradients raise
-``ValueError``.
+summation order.  Nothing here has a derivative: inputs and outputs that need gradients
+(unless under ``torch.no_grad()``) or carry forward-mode tangents raise ``ValueError``.
 """
 
 from __future__ import annotations
@@ -69,6 +69,7 @@ def mx4_dequantize(m: Mx4, dtype: torch.dtype = torch.bfloat16, out: Optional[to
     if given is not None:
         _same("mx4_dequantize", m, out)
     _float_rows("mx4_dequantize", out)
+    _no_grad("mx4_dequantize", out)
     if name == "eager":
         return out.copy_(_eager_values(m))
     _unit_out("mx4_dequantize", out)
@@ -87,7 +88,7 @@ def mx4_rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, slot: Mx4, o
     if name == "hip" and x.is_cuda and hip_attn._require().mx4_rope_fast(x, cos, sin, slot, out) is not None:
         return slot
     _float_rows("mx4_rope", x)
-    _no_grad("mx4_rope", x, cos, sin)
+    _no_grad("mx4_rope", x, cos, sin, out)
     n = x.size(-1)
     if n % 2 != 0:
         raise ValueError(f"RoPE last dim must be even, got {n}")
@@ -148,7 +149,7 @@ def mx4_gemm(a, wt: Mx4, *, relu: bool = False, mul: Optional[torch.Tensor] = No
     if ((a.codes if four else a).get_device() != dev or out.get_device() != dev
             or (mul is not None and mul.get_device() != dev)):
         raise ValueError("mx4_gemm: operands on different devices")
-    _no_grad("mx4_gemm", None if four else a, mul)
+    _no_grad("mx4_gemm", None if four else a, mul, out)
     if name == "eager":
         return out.copy_(_eager_gemm(a, wt, relu, mul))
     _unit_out("mx4_gemm", out)
