@@ -21,6 +21,7 @@ import contextlib
 import ctypes
 import os
 import struct
+import warnings
 from pathlib import Path
 from typing import Optional, Sequence, Tuple
 
@@ -228,12 +229,23 @@ def _load():
 
 _lib, _path = _load()
 
-try:
-    import bdh_bind as _bind  # (beside this file)
-except ImportError as exc:
-    raise ImportError(f"bdh_hip_ext: {exc}; build it with `python bdh-gpu-fast_amd/build.py`") from exc
-_bind.use(*(ctypes.cast(getattr(_lib, f"bdh_mx4_{n}"), ctypes.c_void_p).value for n in (
-    "quantize", "dequantize", "rope", "decode_workspace", "decode", "gemm_workspace", "gemm")))
+
+def _load_bind():
+    """The compiled binding (beside this file), or None, with a warning, where it is not built or was
+    built against another torch or Python: calls then take the ctypes route."""
+    try:
+        import bdh_bind
+
+        bdh_bind.use(*(ctypes.cast(getattr(_lib, f"bdh_mx4_{n}"), ctypes.c_void_p).value for n in (
+            "quantize", "dequantize", "rope", "decode_workspace", "decode", "gemm_workspace", "gemm")))
+    except Exception as exc:
+        warnings.warn(f"bdh_hip_ext: no bdh_bind ({type(exc).__name__}: {exc}); the 4-bit operators' calls take some "
+                      "us more; build it with `python bdh-gpu-fast_amd/build.py`", RuntimeWarning, stacklevel=2)
+        return None
+    return bdh_bind
+
+
+_bind = _load_bind()
 has_hip = True
 # The reference's pybind module reports has_cuda (tril_attn_bind.cpp:34-39); this
 # library has no CUDA path, so a caller probing that attribute sees False.
@@ -1014,7 +1026,7 @@ def mx4_gemm(a: Optional[torch.Tensor], a4, wt, mul: Optional[torch.Tensor], rel
 
 
 # The same through the compiled binding, for arguments that are as the operators want them, on the
-# current device: None where they are not, and nothing has been done then.
+# current device: None where they are not, or there is no binding, and nothing has been done then.
 def _counted(r, what: str):
     global _launches
     if type(r) is int and r != 0:
@@ -1025,26 +1037,36 @@ def _counted(r, what: str):
 
 
 def mx4_quantize_fast(x: torch.Tensor, m) -> Optional[int]:
+    if _bind is None:
+        return None
     i = torch._C._cuda_getDevice()
     return _counted(_bind.quantize(x, m, i, torch._C._cuda_getCurrentRawStream(i)), "mx4_quantize")
 
 
 def mx4_dequantize_fast(m, out: torch.Tensor) -> Optional[int]:
+    if _bind is None:
+        return None
     i = torch._C._cuda_getDevice()
     return _counted(_bind.dequantize(m, out, i, torch._C._cuda_getCurrentRawStream(i)), "mx4_dequantize")
 
 
 def mx4_rope_fast(x, cos, sin, slot, out) -> Optional[int]:
+    if _bind is None:
+        return None
     i = torch._C._cuda_getDevice()
     return _counted(_bind.rope(x, cos, sin, slot, out, i, torch._C._cuda_getCurrentRawStream(i)), "mx4_rope")
 
 
 def mx4_decode_fast(q, k_past, v_past) -> Optional[torch.Tensor]:
+    if _bind is None:
+        return None
     i = torch._C._cuda_getDevice()
     return _counted(_bind.decode(q, k_past, v_past, i, torch._C._cuda_getCurrentRawStream(i)), "mx4_decode")
 
 
 def mx4_gemm_fast(a, wt, relu, mul, out, bf16: bool) -> Optional[torch.Tensor]:
+    if _bind is None:
+        return None
     i = torch._C._cuda_getDevice()
     return _counted(_bind.gemm(a, wt, relu, mul, out, bf16, i, torch._C._cuda_getCurrentRawStream(i)), "mx4_gemm")
 

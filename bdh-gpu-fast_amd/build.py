@@ -89,13 +89,16 @@ def build(jobs: int | None = None, verbose: bool = False) -> Path:
         objs.append(obj)
         cmds.append([cc, *flags, "-c", str(CSRC / src), "-o", str(obj)])
     bind = BIND.with_suffix(".so.tmp")
-    cmds.insert(0, bind_cmd(bind))
-    jobs = jobs or min(len(cmds), os.cpu_count() or 4, 8)
+    jobs = jobs or min(len(cmds) + 1, os.cpu_count() or 4, 8)
     with ThreadPoolExecutor(max_workers=jobs) as ex:
+        binding = ex.submit(lambda: _run(bind_cmd(bind), verbose))
         list(ex.map(lambda c: _run(c, verbose), cmds))
     tmp = LIB.with_suffix(".so.tmp")
     _run([cc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs)], verbose)
+    # the library needs no binding: a failure there comes after it, and leaves none of an earlier build
     os.replace(tmp, LIB)
+    BIND.unlink(missing_ok=True)
+    binding.result()
     os.replace(bind, BIND)
     return LIB
 
