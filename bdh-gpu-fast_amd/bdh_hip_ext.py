@@ -957,12 +957,20 @@ def small_gemm(a: torch.Tensor, b: torch.Tensor, out_dtype: Optional[torch.dtype
     return out
 
 
+def _step_layers(kr, v: torch.Tensor, n: int) -> None:
+    """The library steps through ``n`` layers of both by their strides."""
+    if len(kr.shape) != 5 or v.dim() != 5 or min(kr.shape[0], v.size(0)) < max(n, 1):
+        raise ValueError(f"decode step: kr (L, B, nh, cap, N) and v (L, B, 1, cap, D) with {n} layers wanted, got "
+                         f"{tuple(kr.shape)} and {tuple(v.shape)}")
+
+
 def decode_step(x: torch.Tensor, enc_t: torch.Tensor, encv_t: torch.Tensor, dec: torch.Tensor, cos: torch.Tensor,
                 sin: torch.Tensor, kr: torch.Tensor, v: torch.Tensor, seq_len: int) -> torch.Tensor:
     """All layers of one generate step: x (B, D) fp32 the token's embedding, already in
     layer 0's V slot as bf16; enc_t and encv_t (nh, N, D), dec (nh*N, D) bf16; cos, sin (1, 1, 1, N);
     kr (L, B, nh, cap, N) and v (L, B, 1, cap, D) the bf16 cache with ``seq_len`` rows.
     Returns the last layer's x (B, D); the rows at ``seq_len`` are written."""
+    _step_layers(kr, v, kr.size(0))
     dev = _require_device(x, enc_t, encv_t, dec, cos, sin, kr, v)
     B, D = x.shape
     nh, N, _ = enc_t.shape
@@ -1082,6 +1090,7 @@ def decode_step_mx4(x: torch.Tensor, enc_t, encv_t, dec, cos: torch.Tensor, sin:
     """:func:`decode_step` with ``kr`` (L, B, nh, cap, N), the weights or both in mx4: ``enc_t`` and
     ``encv_t`` (nh, N, D) with ``dec`` (nh*N, D) bf16, or all three as mx4 rows, ``dec`` transposed
     (D, nh*N)."""
+    _step_layers(kr, v, v.size(0))
     four, keys4 = not isinstance(enc_t, torch.Tensor), not isinstance(kr, torch.Tensor)
     dev = _require_device(x, *((m.codes for m in (enc_t, encv_t, dec)) if four else (enc_t, encv_t, dec)), cos, sin,
                           kr.codes if keys4 else kr, v)
