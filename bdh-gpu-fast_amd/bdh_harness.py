@@ -567,7 +567,9 @@ class BDH(nn.Module):
         """Logits (B, T, V) (or (B, 1, V) with ``last_only``) and the loss when ``targets`` is given.
 
         ``weight_dtype="mx4"`` (inference on the HIP path): the encoders and the decoder with the
-        values of their 4-bit form, which a cached step of few tokens reads from memory.
+        values of their 4-bit form, which a cached step of few tokens reads from memory.  It is
+        laid out beside copies of those values in the compute dtype, so it takes more memory than
+        the plain weights, and anew at each call that changes ``weight_dtype``.
 
         With ``cache`` the tokens continue the cached sequence: RoPE positions
         start at ``cache.seq_len`` and every layer's RoPE(x) and V rows are

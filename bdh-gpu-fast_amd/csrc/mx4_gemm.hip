@@ -697,7 +697,7 @@ struct GemmPlan {
 
 // Few rows: splits of K and waves a tile, four waves a CU where K has a wave's four
 // steps for each of them; up to four waves a tile of long rows to make sixteen a CU (3 rows of
-// 4 x 8192 x 13504 128 -> 100 us, but 8 of 4 x 8192 x 1024 12.6 -> 14).
+// 4 x 8192 x 13504 116 -> 88 us, 8 of 4 x 8192 x 8192 71 -> 55, but of 4 x 8192 x 1024 10.7 -> 13.1).
 void few_plan(int64_t H, int64_t M, int64_t N, int64_t K, GemmPlan& p) {
   p.steps = int((mx4_blocks(K) + 1) / 2);
   const int64_t tiles = H * ((M + 31) / 32) * ((N + 31) / 32);
@@ -743,9 +743,10 @@ double tile_plan(int64_t H, int64_t M, int64_t N, int64_t K, GemmPlan& p) {
 
 // The few-row kernel's: 7 us and 240 TFLOP/s in bf16, 500 in mx4, half where rows are long, of
 // whole tiles, and a's bytes at 3 TB/s.  Measured against the tile kernel: bf16 256 x 4096 x 1024
-// 13 us and 23, 1000 x 512 x 2048 14 and 28, 1500 x 256 x 8192 41 and 35, 2048 x 2048 x 2048 69 and
-// 31, 6216 x 32 x 32768 118 and 86 (though it computes 256 columns); mx4 80 x 100 x 256 8 and 19,
-// 64 x 8192 x 4096 13 and 26, 128 x 4096 x 16384 43 and 32, 813 x 8192 x 512 19 and 21.
+// 14 us and 25, 1000 x 512 x 2048 15 and 31, 1500 x 256 x 8192 41 and 35, 2048 x 2048 x 2048 71 and
+// 31, 6216 x 32 x 32768 122 and 97 (though it computes 256 columns); mx4 80 x 100 x 256 7 and 19,
+// 64 x 8192 x 4096 13 and 27, 128 x 4096 x 16384 44 and 30, 813 x 8192 x 512 20 and 21.  It leaves out
+// the weights' bytes, which bound few rows: up to 32 this kernel is taken unasked.
 double few_us(int64_t H, int64_t M, int64_t N, int64_t K, bool a4) {
   const double hmk = double(H) * double(M) * double(K);
   return 7 + std::max(2e-6 * hmk * double(align_up(N, 32)) / ((a4 ? 500 : 240) * (K < 8192 ? 1 : 0.5)),
