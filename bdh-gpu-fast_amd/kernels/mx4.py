@@ -114,6 +114,13 @@ class Mx4:
 
 
 # ------------------------------------------------------------------- eager
+def _pow2(b: torch.Tensor) -> torch.Tensor:
+    """What scale bytes stand for, 2^(b - 127) or NaN, by their bits: on a GPU torch.ldexp goes by a
+    pow that misses powers of two by a step, and codes at a border with it."""
+    b = b.int()
+    return torch.where(b == 0, 0x00400000, torch.where(b == 255, 0x7FC00000, b << 23)).view(torch.float32)
+
+
 def _eager_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     n = x.size(-1)
     y = torch.nn.functional.pad(x.float(), (0, -n % BLOCK)).unflatten(-1, (_blocks(n), BLOCK))
@@ -121,7 +128,7 @@ def _eager_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     bad = ~torch.isfinite(y).all(-1)
     m, e = torch.frexp(torch.where(bad, 0.0, top))  # m 2^e, 0.5 <= m < 1
     e = torch.where(m > 0, e - 3 + (m >= 0.875).int(), -127).clamp(-127, 127)
-    y = torch.ldexp(y, -e.unsqueeze(-1))
+    y = y * _pow2(127 - e).unsqueeze(-1)
     a = y.abs()
     i = torch.where(a < 2, torch.round(2 * a), torch.where(a < 4, torch.round(a) + 2, torch.round(a / 2) + 4))
     i = i.clamp_max(7) + 8 * torch.signbit(y)
@@ -132,9 +139,7 @@ def _eager_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 def _eager_values(m: Mx4) -> torch.Tensor:
     lut = torch.tensor(_GRID + tuple(-v for v in _GRID), device=m.device)
     v = lut[torch.stack((m.codes & 15, m.codes >> 4), -1).flatten(-2).long()].unflatten(-1, (_blocks(m.width), BLOCK))
-    s = torch.ldexp(torch.ones((), device=m.device), m.scales.int() - 127)
-    s = torch.where(m.scales == 255, float("nan"), s)
-    return (v * s.unsqueeze(-1)).flatten(-2)[..., : m.width]
+    return (v * _pow2(m.scales).unsqueeze(-1)).flatten(-2)[..., : m.width]
 
 
 def _eager_rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
