@@ -26,6 +26,7 @@ from pathlib import Path
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 __all__ = [
     "has_hip",
@@ -1085,6 +1086,14 @@ class _StepMx4(ctypes.Structure):
         ("scale_layer", ctypes.c_int64)]
 
 
+def _no_derivative(what: str, ts: Sequence[torch.Tensor]) -> None:
+    """Operands that need gradients, or carry tangents where a level of forward mode is open."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        raise ValueError(f"{what} has no derivative: call it under torch.no_grad() or detach its operands")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise ValueError(f"{what} has no derivative: call it on the primal tensors")
+
+
 def decode_step_mx4(x: torch.Tensor, enc_t, encv_t, dec, cos: torch.Tensor, sin: torch.Tensor, kr, v: torch.Tensor,
                     seq_len: int) -> torch.Tensor:
     """:func:`decode_step` with ``kr`` (L, B, nh, cap, N), the weights or both in mx4: ``enc_t`` and
@@ -1092,6 +1101,7 @@ def decode_step_mx4(x: torch.Tensor, enc_t, encv_t, dec, cos: torch.Tensor, sin:
     (D, nh*N)."""
     _step_layers(kr, v, v.size(0))
     four, keys4 = not isinstance(enc_t, torch.Tensor), not isinstance(kr, torch.Tensor)
+    _no_derivative("decode_step_mx4", [t for t in (x, enc_t, encv_t, dec, cos, sin, kr, v) if isinstance(t, torch.Tensor)])
     dev = _require_device(x, *((m.codes for m in (enc_t, encv_t, dec)) if four else (enc_t, encv_t, dec)), cos, sin,
                           kr.codes if keys4 else kr, v)
     B, D = x.shape
